@@ -264,7 +264,8 @@ int pm_nvfp4_prepare_search(const uint8_t *w, const float *s, const float *impor
  * x bf16 [T, K], a bf16 [N, R, K], b bf16 [N, O, R], adapter i32 [T], scale f32 [N] (NULL: 1), base bf16 [T, O] (NULL:
  * 0), out bf16 [T, O] (may be base itself, with its row distance; else it overlaps no input). ld*: elements from one
  * row to the next, a multiple of 8. K, O and R are multiples of 8, R <= 128, N <= 1024, T <= 2^24, K and O <= 2^20.
- * The sums over K and R are fp32, the R values between them are kept to 16 significant bits, out is rounded once.
+ * The sums over K and R are fp32, the R values between them are kept to 16 significant bits, out is rounded once; results are
+ * infinite or NaN where the formula's are (values between the products below 2^-134 count as 0).
  * Results do not depend on the other rows' order, and repeat bit for bit.
  *
  * pm_lora_grad: from dy bf16 [T, O], the gradient of out:

@@ -61,6 +61,39 @@ __device__ __forceinline__ void split2(float v, __nv_bfloat16* hi, __nv_bfloat16
     *lo = fabsf(f) <= 3.4e38f ? __float2bfloat16_rn(v - f) : __float2bfloat16_rn(0.0f);
 }
 
+// An infinite operand times a low half is NaN (a half of 0) or infinite of the other sign. So where the sum over both halves is
+// not finite, the high halves' alone is the result: a high half has its value's sign, and is 0 only where the value is (or
+// below 2^-134). The kernels look at what they have made and, where something is not finite, make it once more.
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466e38f; }
+__device__ __forceinline__ float both_halves(float both, float high) { return finite(both) ? both : high; }
+// Whether one of a warp's sums is not finite.
+__device__ __forceinline__ bool any_not_finite(const float (&v)[4]) {
+    const float z = fmaf(v[0], 0.0f, v[1] * 0.0f) + fmaf(v[2], 0.0f, v[3] * 0.0f);
+    return __any_sync(0xffffffffu, !(z == 0.0f)) != 0;
+}
+template <int M>
+__device__ __forceinline__ bool any_not_finite(const float (&v)[M][4]) {
+    float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[e] = fmaf(v[i][e], 0.0f, z[e]);
+    return any_not_finite(z);
+}
+// The same for results, pairs of bf16, collected one by one.
+struct Unusual {
+    __nv_bfloat162 z[2];
+    __device__ __forceinline__ Unusual() : z{__nv_bfloat162(0.0f, 0.0f), __nv_bfloat162(0.0f, 0.0f)} {}
+    __device__ __forceinline__ void see(uint32_t pair, int i) {
+        z[i] = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&pair), __nv_bfloat162(0.0f, 0.0f), z[i]);
+    }
+    __device__ __forceinline__ void see(const uint4& v) { see(v.x, 0), see(v.y, 1), see(v.z, 0), see(v.w, 1); }
+    __device__ __forceinline__ bool any() const {
+        const __nv_bfloat162 s = __hadd2(z[0], z[1]);
+        return __any_sync(0xffffffffu, (*reinterpret_cast<const uint32_t*>(&s) & 0x7fff7fffu) != 0u) != 0;
+    }
+};
+
 // Eight values as their halves.
 __device__ __forceinline__ void split8(const float (&v)[8], uint4* hi, uint4* lo) {
     __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(hi);

@@ -237,6 +237,21 @@ __global__ void __launch_bounds__(kFewThreads) lora_fused_kernel(const FewArgs g
 #pragma unroll
                 for (int i = 0; i < 4; ++i) mma16816(d[i], h0.x, h1.x, h0.y, h1.y, wb[i][q].x, wb[i][q].y);
             }
+        if (any_not_finite(d)) {  // once more (here: a call would cost registers, of which four CTAs to an SM have 64 a thread)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (!any_not_finite(d[i])) continue;  // a tile at a time
+                float high[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int q = 0; q < kChunks; ++q) {
+                    const bf16* at = hs + gr * kLdh + q * 16 + c * 4;
+                    const uint2 h0 = *reinterpret_cast<const uint2*>(at), h1 = *reinterpret_cast<const uint2*>(at + 8 * kLdh);
+                    mma16816(high, h0.x, h1.x, h0.y, h1.y, wb[i][q].x, wb[i][q].y);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) d[i][e] = both_halves(d[i][e], high[e]);
+            }
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             uint4 o = y[h];

@@ -68,6 +68,11 @@ __device__ __forceinline__ void ldmatrix_trans(uint32_t addr, uint32_t (&r)[4]) 
 }
 __device__ __forceinline__ uint32_t lower(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
 __device__ __forceinline__ uint32_t upper(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
+// Two bf16: those of `stored` that are finite, else those of `other`.
+__device__ __forceinline__ uint32_t keep_finite(uint32_t stored, uint32_t other) {
+    const uint32_t m = ((stored & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((stored & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+    return (other & m) | (stored & ~m);
+}
 // Value i of 8 columns, of two neighbouring rows.
 __device__ __forceinline__ void pair_rows(const uint4& p, const uint4& q, uint32_t (&out)[8]) {
     out[0] = lower(p.x, q.x), out[1] = upper(p.x, q.x), out[2] = lower(p.y, q.y), out[3] = upper(p.y, q.y);
@@ -228,6 +233,20 @@ struct RowsOfDx {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) mma16816(d[i], f.x, f.y, f.z, f.w, a.w[q][0][i], a.w[q][1][i]);
             }
+        if (any_not_finite(d)) {  // once more
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (!any_not_finite(d[i])) continue;  // a tile at a time: registers of one
+                float high[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int q = 0; q < RankRows<NT>::kSteps; ++q) {
+                    const uint4 f = frag(0, q);
+                    mma16816(high, f.x, f.y, f.z, f.w, a.w[q][0][i], a.w[q][1][i]);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) d[i][e] = both_halves(d[i][e], high[e]);
+            }
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -243,23 +262,29 @@ struct RowsOfDx {
     }
 };
 
-// 64 columns of dA (is_a) or dB, summed over tiles from, from + step, .. of 16 rows: row(i) is the adapter's row i or -1,
+struct WeightSide {
+    const bf16* src;  // x or dy
+    long ld;
+    bf16* out;        // the adapter's dA [R][width] or dB [width][R]
+    int width, R;
+    bool is_a;
+};
+// 64 columns of dA or dB, summed over tiles from, from + step, .. of 16 rows: row(i) is the adapter's row i or -1,
 // frag(tile, half, step) the halves of d or h with their rows as the contraction. GLOBAL: both come from global memory, and are
 // asked for ahead like the rows themselves (one tile; with four the warps' registers left one CTA an SM: 333 rows 13.5 us, not
 // 11.8).
-// acc, dA: [steps of 16 ranks][8 tiles of columns]; dB: [steps of 16 ranks][4 tiles
-// of 16 columns][2 tiles of 8 ranks].
+// acc, dA: [steps of 16 ranks][8 tiles of columns]; dB: [steps of 16 ranks][4 tiles of 16 columns][2 tiles of 8 ranks].
+// HIGH: of the high halves alone, after a store of sums of both that were not all finite; those that were stay.
 template <int NT, bool GLOBAL>
 struct WeightBlock {
     static constexpr int kSteps = NT == 1 ? 1 : NT / 2;
     float acc[kSteps * 8][4];
-    template <class Row, class Frag>
-    __device__ __forceinline__ void sum(const GradFewArgs& g, bool is_a, int block, int from, int step, int tiles, Row row,
-                                        Frag frag) {
+    template <bool HIGH, class Row, class Frag>
+    __device__ __forceinline__ void sum(const WeightSide& s, int block, int from, int step, int tiles, Row row, Frag frag) {
         const int lane = threadIdx.x & 31, gr = lane >> 2, c = lane & 3;
-        const int width = is_a ? g.K : g.O, col = block * 64 + gr * 8;
-        const bf16* src = is_a ? g.x : g.dy;
-        const long ld = is_a ? g.ldx : g.lddy;
+        const int width = s.width, col = block * 64 + gr * 8;
+        const bf16* src = s.src;
+        const long ld = s.ld;
         const uint4 zero = make_uint4(0, 0, 0, 0);
         int id[4];
         uint4 v[4], f[2][kSteps];
@@ -274,7 +299,7 @@ struct WeightBlock {
                 v[e] = id[e] >= 0 && col < width ? *reinterpret_cast<const uint4*>(src + (long)id[e] * ld + col) : zero;
             if (!GLOBAL) return;
 #pragma unroll
-            for (int hl = 0; hl < 2; ++hl)
+            for (int hl = 0; hl < (HIGH ? 1 : 2); ++hl)
 #pragma unroll
                 for (int q = 0; q < kSteps; ++q) f[hl][q] = tile < tiles ? frag(tile, hl, q) : zero;
             number(tile + step);
@@ -291,11 +316,11 @@ struct WeightBlock {
             pair_rows(v[2], v[3], hi);
             if (!GLOBAL) ask(tile + step);
 #pragma unroll
-            for (int hl = 0; hl < 2; ++hl)
+            for (int hl = 0; hl < (HIGH ? 1 : 2); ++hl)
 #pragma unroll
                 for (int q = 0; q < kSteps; ++q) {
                     const uint4 r = GLOBAL ? f[hl][q] : frag(tile, hl, q);
-                    if (is_a) {
+                    if (s.is_a) {
 #pragma unroll
                         for (int i = 0; i < 8; ++i) mma16816(acc[q * 8 + i], r.x, r.y, r.z, r.w, lo[i], hi[i]);
                     } else {
@@ -310,10 +335,10 @@ struct WeightBlock {
             if (GLOBAL) ask(tile + step);
         }
     }
-    __device__ __forceinline__ void store(const GradFewArgs& g, bool is_a, int block, int n) const {
+    template <bool HIGH>
+    __device__ __forceinline__ void store(const WeightSide& s, int block) const {
         const int lane = threadIdx.x & 31, gr = lane >> 2, c = lane & 3;
-        if (is_a) {
-            bf16* da = g.da + (long)n * g.R * g.K;
+        if (s.is_a) {
 #pragma unroll
             for (int q = 0; q < kSteps; ++q)
 #pragma unroll
@@ -322,23 +347,45 @@ struct WeightBlock {
                     float f[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) f[i] = acc[q * 8 + i][k];
-                    if (r < g.R && o < g.K) *reinterpret_cast<uint4*>(da + (long)r * g.K + o) = pack8(f);
+                    if (r < s.R && o < s.width) {
+                        uint4* p = reinterpret_cast<uint4*>(s.out + (long)r * s.width + o);
+                        uint4 v = pack8(f);
+                        if (HIGH) {
+                            const uint4 was = *p;
+                            v = make_uint4(keep_finite(was.x, v.x), keep_finite(was.y, v.y), keep_finite(was.z, v.z),
+                                           keep_finite(was.w, v.w));
+                        }
+                        *p = v;
+                    }
                 }
-        } else if (block * 64 + gr * 8 < g.O) {
-            bf16* db = g.db + ((long)n * g.O + block * 64 + gr * 8) * g.R;
+        } else if (block * 64 + gr * 8 < s.width) {
+            bf16* db = s.out + (long)(block * 64 + gr * 8) * s.R;
 #pragma unroll
             for (int q = 0; q < kSteps; ++q)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {  // tile i / 2 of 16 columns, of its rank tile i % 2
                     const int r = q * 16 + (i & 1) * 8 + 2 * c;
-                    if (r < g.R) {
-                        bf16* p = db + (i >> 1) * 2 * g.R + r;
-                        *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(acc[q * 8 + i][0], acc[q * 8 + i][1]);
-                        *reinterpret_cast<__nv_bfloat162*>(p + g.R) =
-                            __floats2bfloat162_rn(acc[q * 8 + i][2], acc[q * 8 + i][3]);
+                    if (r < s.R) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            uint32_t* p = reinterpret_cast<uint32_t*>(db + ((i >> 1) * 2 + h) * s.R + r);
+                            const __nv_bfloat162 two = __floats2bfloat162_rn(acc[q * 8 + i][2 * h], acc[q * 8 + i][2 * h + 1]);
+                            uint32_t v = *reinterpret_cast<const uint32_t*>(&two);
+                            if (HIGH) v = keep_finite(*p, v);
+                            *p = v;
+                        }
                     }
                 }
         }
+    }
+    // What is not finite once more.
+    template <class Row, class Frag>
+    static __device__ __noinline__ void again(const bf16* src, long ld, bf16* out, int width, int R, bool is_a, int block,
+                                              int tiles, Row row, Frag frag) {
+        const WeightSide s{src, ld, out, width, R, is_a};
+        WeightBlock w;
+        w.template sum<true>(s, block, 0, 1, tiles, row, frag);
+        w.template store<true>(s, block);
     }
 };
 
@@ -481,10 +528,15 @@ __global__ void __launch_bounds__(grad_threads<NT>()) lora_grad_few_kernel(const
             const int block = is_a ? it : it - kb;
             const bf16* from = is_a ? dh : hh;
             WeightBlock<NT, false> w;
-            w.sum(g, is_a, block, 0, 1, tiles, [&](int i) { return list[i]; }, [&](int tile, int hl, int q) {
-                return frag_trans<kLd>(from + hl * half + tile * 16 * kLd + q * 16);
-            });
-            w.store(g, is_a, block, n);
+            const WeightSide s{is_a ? g.x : g.dy, is_a ? g.ldx : g.lddy, is_a ? da : db, is_a ? g.K : g.O, g.R, is_a};
+            auto row = [&](int i) { return list[i]; };
+            auto frag = [&](int tile, int hl, int q) { return frag_trans<kLd>(from + hl * half + tile * 16 * kLd + q * 16); };
+            w.template sum<false>(s, block, 0, 1, tiles, row, frag);
+            w.template store<false>(s, block);
+            if (any_not_finite(w.acc)) {  // once more
+                w.template sum<true>(s, block, 0, 1, tiles, row, frag);
+                w.template store<true>(s, block);
+            }
         } else {
             const int block = (it - kb - ob) % kb;
             RankRows<NT> w;
@@ -493,7 +545,7 @@ __global__ void __launch_bounds__(grad_threads<NT>()) lora_grad_few_kernel(const
                 RowsOfDx r;
                 r.t[0] = list[tile * 16 + gr], r.t[1] = list[tile * 16 + 8 + gr];
                 r.load(g, block);
-                r.finish<NT>(g, block, w, [&](int hl, int q) {
+                r.finish<NT>(g, block, w, [dh, half, tile](int hl, int q) {
                     return frag_rows<kLd>(dh + hl * half + tile * 16 * kLd + q * 16);
                 });
             }
@@ -579,8 +631,11 @@ __global__ void __launch_bounds__(kGroupThreads, 2) lora_grad_finish_kernel(cons
         pdl_trigger();
         const uint4* f = frags + ((long)first * 6 + (is_a ? 0 : 4)) * kSteps * 32 + lane;
         WeightBlock<NT, true> w;
-        w.sum(g, is_a, block, part, SPLIT, tiles, [&](int i) { return i < rows ? __ldcg(at + i) : -1; },
-              [&](int tile, int hl, int q) { return __ldcg(f + ((long)tile * 6 * kSteps + hl * kSteps + q) * 32); });
+        auto row = [at, rows](int i) { return i < rows ? __ldcg(at + i) : -1; };
+        auto frag = [f](int tile, int hl, int q) { return __ldcg(f + ((long)tile * 6 * kSteps + hl * kSteps + q) * 32); };
+        const WeightSide s{is_a ? g.x : g.dy, is_a ? g.ldx : g.lddy, (is_a ? g.da : g.db) + (long)n * g.R * (is_a ? g.K : g.O),
+                           is_a ? g.K : g.O, g.R, is_a};
+        w.template sum<false>(s, block, part, SPLIT, tiles, row, frag);
         if (SPLIT > 1) {
             float4* mine = red + warp / SPLIT * (SPLIT - 1) * kAcc * 32 + lane;
             if (part > 0) {
@@ -597,7 +652,9 @@ __global__ void __launch_bounds__(kGroupThreads, 2) lora_grad_finish_kernel(cons
                     w.acc[i][0] += v.x, w.acc[i][1] += v.y, w.acc[i][2] += v.z, w.acc[i][3] += v.w;
                 }
         }
-        if (live) w.store(g, is_a, block, n);
+        if (!live) return;
+        w.template store<false>(s, block);
+        if (any_not_finite(w.acc)) w.again(s.src, s.ld, s.out, s.width, s.R, is_a, block, tiles, row, frag);
         return;
     }
     const int per = (kb + kGroupWarps - 1) / kGroupWarps;
@@ -616,7 +673,7 @@ __global__ void __launch_bounds__(kGroupThreads, 2) lora_grad_finish_kernel(cons
     pdl_trigger();
     if (!live) return;
     const uint4* f = frags + ((long)group * 6 + 2) * kSteps * 32 + lane;
-    r.finish<NT>(g, block, w, [&](int hl, int q) { return __ldcg(f + (hl * kSteps + q) * 32); });
+    r.finish<NT>(g, block, w, [f](int hl, int q) { return __ldcg(f + (hl * kSteps + q) * 32); });
 }
 
 template <int NT, int SPLIT>

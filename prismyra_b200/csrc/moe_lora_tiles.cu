@@ -581,7 +581,8 @@ __global__ void __launch_bounds__(kOuterThreads, 1)
                         if (q + e >= g.R) break;
                         float v[8];
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) v[k] = __uint_as_float(a[e + k]) + __uint_as_float(b[e + k]);
+                        for (int k = 0; k < 8; ++k)
+                            v[k] = both_halves(__uint_as_float(a[e + k]) + __uint_as_float(b[e + k]), __uint_as_float(a[e + k]));
                         if (whole) {
                             store_ranks(g, is_a, n, tile * kLoraCols + c, q + e, v);
                         } else {
@@ -659,7 +660,34 @@ constexpr int kUpStages = 3;
 constexpr int kUpThreads = 384;   // warps 0-7: base in, results out; 8: MMA; 9: TMA; 10, 11: rows without an adapter, shared
                                   // gradient tiles
 
+// A warp's 32 x 32 results in its stage of shared memory (a row per lane, 16-byte pieces as the kernel lays them), once more where
+// they are not finite and their column's weights hold an infinity: h this lane's row of high halves, base its row (null: 0), first
+// the warp's first column. by_rank: w is [R][width], else [width][R]. The hidden rows are there: their products are.
+__device__ __noinline__ void again(uint8_t* stage, const bf16* h, const bf16* w, int by_rank, int R, int width, int first,
+                                   const bf16* base) {
+    const int lane = threadIdx.x & 31;
+    const long column = by_rank ? 1 : R, rank = by_rank ? width : 1;
+    bool inf = false;
+    if (first + lane < width)
+#pragma unroll 8
+        for (int r = 0; r < R; ++r)
+            inf |= (__bfloat16_as_ushort(w[(first + lane) * column + r * rank]) & 0x7fffu) == 0x7f80u;
+    for (uint32_t todo = __ballot_sync(0xffffffffu, inf); todo != 0; todo &= todo - 1) {
+        const int j = __ffs(todo) - 1;
+        const bf16* p = w + (first + j) * column;
+        float s = 0.0f;
+#pragma unroll 8
+        for (int r = 0; r < R; ++r)
+            s = fmaf(__bfloat162float(__ldcg(h + r)), __bfloat162float(p[r * rank]), s);
+        if (base != nullptr) s += __bfloat162float(__ldcg(base + first + j));
+        bf16* o = reinterpret_cast<bf16*>(stage + lane * 64 + (((j >> 3) ^ ((lane >> 1) & 3)) << 4)) + (j & 7);
+        if (!finite(__bfloat162float(*o))) *o = __float2bfloat16_rn(s);
+    }
+}
+
 struct UpArgs {
+    const bf16* h;
+    const bf16* w;
     const bf16* base;
     long ldbase;
     bf16* out;
@@ -897,6 +925,7 @@ __global__ void __launch_bounds__(kUpThreads, 2)
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&tail->aempty[buf]));
+            Unusual unusual;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 y[q].x = add_bf16x2(y[q].x, __uint_as_float(r[q * 8]), __uint_as_float(r[q * 8 + 1]));
@@ -904,6 +933,12 @@ __global__ void __launch_bounds__(kUpThreads, 2)
                 y[q].z = add_bf16x2(y[q].z, __uint_as_float(r[q * 8 + 4]), __uint_as_float(r[q * 8 + 5]));
                 y[q].w = add_bf16x2(y[q].w, __uint_as_float(r[q * 8 + 6]), __uint_as_float(r[q * 8 + 7]));
                 *reinterpret_cast<uint4*>(at + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) = y[q];
+                unusual.see(y[q]);
+            }
+            if (unusual.any()) {
+                const int slot = block * kLoraTile + quarter * 32 + lane, row = __ldcg(g.rows + slot);
+                again(at, g.h + (long)slot * 2 * Rp, g.w + (long)__ldcg(g.adapter + block) * g.R * g.width, g.by_rank, g.R,
+                      g.width, tile * kUpCols + half * 32, row < 0 || g.base == nullptr ? nullptr : g.base + (long)row * g.ldbase);
             }
             __syncwarp();
             const int col = tile * kUpCols;
@@ -1032,6 +1067,8 @@ cudaError_t launch_lora_up(const LoraUp& u, const int32_t* adapter, const LoraPl
         return cudaErrorInvalidValue;
     UpArgs a;
     memset(&a, 0, sizeof(a));
+    a.h = u.h;
+    a.w = u.w;
     a.base = u.base;
     a.ldbase = u.ldbase;
     a.out = u.out;
