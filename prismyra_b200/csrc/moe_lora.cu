@@ -602,6 +602,7 @@ int pm_lora_grad(const void* dy, int64_t lddy, const void* x, int64_t ldx, const
     if (T == 0) {
         cudaError_t e = cudaMemsetAsync(da, 0, (size_t)N * R * K * 2, s);
         if (e == cudaSuccess) e = cudaMemsetAsync(db, 0, (size_t)N * R * O * 2, s);
+        if (e == cudaSuccess && !few) e = cudaMemsetAsync(workspace, 0, 16, s);  // the status
         return status_of(e);
     }
     const LoraGradFew f{(const bf16*)dy, (const bf16*)x, (const bf16*)a, (const bf16*)b, lddy, ldx, adapter, scale,

@@ -246,14 +246,22 @@ class AdaptedProjection(nn.Module):
         if scale is not None and tuple(scale.shape) != (N,):
             raise AdapterError(f"scale must hold {N} values")
 
-    def forward(self, x: torch.Tensor, adapter: torch.Tensor):
+    def workspaces(self, rows: int) -> list:
+        """Scratch to keep for forwards of ``rows`` rows, one for each part (None: no adapters there), whose kernels' status
+        ``ops.read_status`` can then be asked for."""
+        parts = [getattr(self, f"a{i}") for i in range(len(self.sizes))]
+        return [a if a is None else ops.lora_workspace(rows, self.in_features, size, a.shape[1], a.shape[0], device=a.device)
+                for a, size in zip(parts, self.sizes)]
+
+    def forward(self, x: torch.Tensor, adapter: torch.Tensor, workspaces: list | None = None):
         rows = x.reshape(-1, self.in_features).contiguous()
         out = self.inner(rows)
         parts = list(out) if isinstance(out, tuple) else [out]
         for i, y in enumerate(parts):
             a = getattr(self, f"a{i}")
             if a is not None:
-                ops.lora(rows, a, getattr(self, f"b{i}"), adapter, getattr(self, f"scale{i}"), base=y, out=y)
+                ops.lora(rows, a, getattr(self, f"b{i}"), adapter, getattr(self, f"scale{i}"), base=y, out=y,
+                         workspace=None if workspaces is None else workspaces[i])
         parts = [y.reshape(*x.shape[:-1], y.shape[-1]) for y in parts]
         return tuple(parts) if isinstance(out, tuple) else parts[0]
 

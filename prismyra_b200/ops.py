@@ -381,7 +381,7 @@ def forward_fp8_host(x_host: torch.Tensor, w1: torch.Tensor, w1_s: torch.Tensor,
 
 
 def read_status(workspace: torch.Tensor) -> None:
-    """Synchronise and raise if a kernel of the last forward on this workspace gave up on a bounded wait."""
+    """Synchronise and raise if a kernel of the last call on this workspace gave up on a bounded wait."""
     _lib.call("pm_moe_read_status", _p(workspace), _stream(workspace.device))
 
 
@@ -696,39 +696,64 @@ def _base_and_out(base, out, x, width, T, dev):
 
 
 @functools.lru_cache(maxsize=4096)
-def _lora_workspace(sizes: tuple, grad: int) -> int:
+def _lora_bytes(sizes: tuple, grad: int) -> int:
     return int(_lib.load().pm_lora_workspace_bytes(*sizes, grad))
 
 
+def lora_workspace(T: int, K: int, O: int, R: int, N: int, grad: bool = False, device=None) -> torch.Tensor:
+    """A workspace to keep for :func:`lora` (grad: :func:`lora_grad`) calls of T rows x [T, K], adapters a [N, R, K] and
+    b [N, O, R], whose kernels' status can then be asked with :func:`read_status`."""
+    return torch.zeros(max(_lora_bytes((T, K, O, R, N), int(grad)), 16), dtype=torch.uint8, device=device or "cuda")
+
+
+def _lora_scratch(workspace: torch.Tensor | None, n: int, x: torch.Tensor, dev: int):
+    """The tensor that holds a call's n bytes of scratch (None: it needs none), and its address. A caller's own begins
+    with the status word, which calls without scratch, whose kernels wait for nothing, leave at 0."""
+    if workspace is None:
+        workspace = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+        return workspace, workspace.data_ptr() if n else None
+    if workspace.dtype != torch.uint8 or workspace.dim() != 1:
+        raise ValueError("workspace must be a uint8 vector")
+    at = _fits(workspace, "workspace", torch.uint8, workspace.shape, dev)
+    if workspace.numel() < max(n, 16) or at % 16:
+        raise ValueError(f"workspace must hold {max(n, 16)} bytes from a 16-byte boundary on, got {workspace.numel()}")
+    if n == 0:
+        workspace[:16].zero_()
+    return workspace, at
+
+
 def lora(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter: torch.Tensor, scale: torch.Tensor | None = None,
-         base: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+         base: torch.Tensor | None = None, out: torch.Tensor | None = None,
+         workspace: torch.Tensor | None = None) -> torch.Tensor:
     """The low-rank adapters of many requests beside a projection they share: for every row t of x [..., K] bf16
     out[t] = base[t] + scale[n] * (x[t] a[n]^T) b[n]^T with n = adapter[t], and out[t] = base[t] where n is outside
     [0, N) (-1: no adapter).  a [N, R, K], b [N, O, R] bf16; adapter int32, one value for each row, in any order; scale
     fp32 [N] (None: 1); base [..., O] bf16 (None: 0), e.g. :func:`fp8_linear`'s or the router's output.  ``out`` may
     be ``base`` itself; otherwise it overlaps no input.  x, base and out may be column slices of wider matrices.
     K, O and R are multiples of 8, R <= 128, N <= 1024; adapters of a smaller rank are padded with zeros.
-    fp32 sums, one rounding; a row's result does not depend on the other rows' order."""
+    fp32 sums, one rounding; a row's result does not depend on the other rows' order.  ``workspace``: scratch of the
+    caller's (:func:`lora_workspace`; not shared by calls that may run at the same time), for :func:`read_status`."""
     px, ldx, pa, pb, pi, ps, sizes, dev = _adapter_args(x, a, b, adapter, scale)
     T, O = sizes[0], sizes[2]
     py, ldy, po, ldo, out = _base_and_out(base, out, x, O, T, dev)
+    n = _lora_bytes(sizes, 0) if T else 0  # 0 for few rows
+    ws, pw = _lora_scratch(workspace, n, x, dev)
     if T == 0:
         return out
     if po == px:
         raise ValueError("out must not be x")
-    n = _lora_workspace(sizes, 0)  # 0 for few rows
-    ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-    _call_on(dev, "pm_lora", px, ldx, pa, pb, pi, ps, py, ldy, po, ldo, *sizes, ws.data_ptr() if n else None, n)
+    _call_on(dev, "pm_lora", px, ldx, pa, pb, pi, ps, py, ldy, po, ldo, *sizes, pw, n)
     return out
 
 
 def lora_grad(dy: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter: torch.Tensor,
-              scale: torch.Tensor | None = None, base: torch.Tensor | None = None, out: torch.Tensor | None = None):
+              scale: torch.Tensor | None = None, base: torch.Tensor | None = None, out: torch.Tensor | None = None,
+              workspace: torch.Tensor | None = None):
     """The gradients of :func:`lora` for dy [..., O] bf16, the gradient of its result: (dx, da, db) in bf16, shaped
     like x, a and b.  dx = base + scale[n] * (dy b[n]) a[n], where ``base`` [..., K] is the gradient of x so far (through
     the shared projection; None: 0); da and db are sums over each adapter's rows, 0 for an adapter without rows.
     ``out`` takes dx and may be ``base`` itself.  The gradient of lora's own base is dy.  Sums are fp32 in a fixed
-    order: the same call gives the same bits."""
+    order: the same call gives the same bits.  ``workspace`` as in :func:`lora` (``lora_workspace(..., grad=True)``)."""
     px, ldx, pa, pb, pi, ps, sizes, dev = _adapter_args(x, a, b, adapter, scale)
     T, K, O = sizes[:3]
     pg, _, ldg = _rows(dy, "dy", O, dev, T)
@@ -737,10 +762,10 @@ def lora_grad(dy: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tenso
         raise ValueError("out must be neither x nor dy")
     da, db = torch.empty_like(a), torch.empty_like(b)
     _need(T <= 1 << 24, "unsupported number of rows")
-    n = _lora_workspace(sizes, 1)  # 0 for few rows
-    ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+    n = _lora_bytes(sizes, 1)  # 0 for few rows
+    ws, pw = _lora_scratch(workspace, n, x, dev)
     _call_on(dev, "pm_lora_grad", pg, ldg, px, ldx, pa, pb, pi, ps, py, ldy, po, ldo, da.data_ptr(), db.data_ptr(), *sizes,
-             ws.data_ptr() if n else None, n)
+             pw, n)
     return out, da, db
 
 
