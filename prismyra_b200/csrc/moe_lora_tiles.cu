@@ -786,8 +786,10 @@ __global__ void __launch_bounds__(kUpThreads, 2)
                 if (++wst == kUpStages) { wst = 0; wphase ^= 1u; }
             };
             for (int i = 0; i < min(count, kUpStages); ++i) load_w(i);
-            if (!AFTER_OUTER) pdl_wait();  // the hidden rows
-            pdl_trigger();
+            if (!AFTER_OUTER) {
+                pdl_wait();  // the hidden rows
+                pdl_trigger();
+            }
             fence_proxy_async_global();  // they were written with plain stores
             int hblock = -1, hloads = 0, block = block0, tile = tile0;
             for (int i = 0; i < count; ++i, next_tile(block, tile)) {
@@ -851,6 +853,7 @@ __global__ void __launch_bounds__(kUpThreads, 2)
             for (int i = (warp - 10) * 32 + lane; i <= g.N; i += 64) units[i] = __ldcg(g.sums.units + i);
             named_bar_sync(1, 64);
             pdl_wait();  // the partial sums
+            pdl_trigger();
             sum_shared_tiles(g.sums, units, g.sum_ctas, spare, spares, lane);
         }
     } else {
