@@ -666,10 +666,13 @@ def _adapter_args(x, a, b, adapter, scale):
     O = b.shape[1]
     if not (N > 0 and R > 0 and K > 0 and O > 0):
         raise ValueError("a and b must not be empty")
-    if K % 8 or O % 8 or R % 8 or R > 128 or N > 1024:
-        raise ValueError(f"unsupported adapters N={N} R={R} K={K} O={O} (need K, O, R % 8 == 0, R <= 128, N <= 1024)")
+    if K % 8 or O % 8 or R % 8 or R > 128 or N > 1024 or K > 1 << 20 or O > 1 << 20:
+        raise ValueError(f"unsupported adapters N={N} R={R} K={K} O={O} (need K, O, R % 8 == 0, K, O <= 2^20, R <= 128, "
+                         "N <= 1024)")
     dev = x.get_device()
     px, T, ldx = _rows(x, "x", K, dev)
+    if T > 1 << 24:
+        raise ValueError(f"at most 2^24 rows, got {T}")
     pa = _fits(a, "a", torch.bfloat16, (N, R, K), dev)
     pb = _fits(b, "b", torch.bfloat16, (N, O, R), dev)
     if pa % 16 or pb % 16:
@@ -730,7 +733,7 @@ def lora(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter: torch.Tenso
     [0, N) (-1: no adapter).  a [N, R, K], b [N, O, R] bf16; adapter int32, one value for each row, in any order; scale
     fp32 [N] (None: 1); base [..., O] bf16 (None: 0), e.g. :func:`fp8_linear`'s or the router's output.  ``out`` may
     be ``base`` itself; otherwise it overlaps no input.  x, base and out may be column slices of wider matrices.
-    K, O and R are multiples of 8, R <= 128, N <= 1024; adapters of a smaller rank are padded with zeros.
+    K, O and R are multiples of 8, R <= 128, N <= 1024, at most 2^24 rows; adapters of a smaller rank are padded with zeros.
     fp32 sums, one rounding; a row's result does not depend on the other rows' order.  ``workspace``: scratch of the
     caller's (:func:`lora_workspace`; not shared by calls that may run at the same time), for :func:`read_status`."""
     px, ldx, pa, pb, pi, ps, sizes, dev = _adapter_args(x, a, b, adapter, scale)
@@ -761,7 +764,6 @@ def lora_grad(dy: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tenso
     if T > 0 and (po == px or po == pg):
         raise ValueError("out must be neither x nor dy")
     da, db = torch.empty_like(a), torch.empty_like(b)
-    _need(T <= 1 << 24, "unsupported number of rows")
     n = _lora_bytes(sizes, 1)  # 0 for few rows
     ws, pw = _lora_scratch(workspace, n, x, dev)
     _call_on(dev, "pm_lora_grad", pg, ldg, px, ldx, pa, pb, pi, ps, py, ldy, po, ldo, da.data_ptr(), db.data_ptr(), *sizes,
@@ -789,6 +791,8 @@ def _router_args(logits, topk_ids, valid):
     k = topk_ids.shape[1]
     if not (1 <= E <= 256 and 1 <= k <= 16 and k <= E):
         raise ValueError(f"unsupported router E={E} k={k} (need k <= 16, k <= E <= 256)")
+    if T >= 1 << 31:
+        raise ValueError(f"fewer than 2^31 rows, got {T}")
     _cuda(logits, "logits", (torch.bfloat16, torch.float32))
     dev = logits.get_device()
     pi = _fits(topk_ids, "topk_ids", torch.int32, (T, k), dev)
