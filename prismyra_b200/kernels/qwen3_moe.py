@@ -203,7 +203,8 @@ class AdaptedProjection(nn.Module):
 
     ``inner`` is an :class:`Fp8Linear` with ``adapters`` = (a [N, R, in] bf16, b [N, out, R] bf16[, scale fp32 [N]]), or
     a :class:`FusedDenseProjection` with one such tuple, or None, for each of its parts (N the same in all); its
-    forward then returns the parts' outputs.  ``adapter`` holds one int32 for each row of x."""
+    forward then returns the parts' outputs.  ``adapter`` holds one int32 for each row of x.  For serving: no gradient goes
+    through it."""
 
     def __init__(self, inner: nn.Module, adapters):
         super().__init__()
@@ -254,7 +255,7 @@ class AdaptedProjection(nn.Module):
                 for a, size in zip(parts, self.sizes)]
 
     def forward(self, x: torch.Tensor, adapter: torch.Tensor, workspaces: list | None = None):
-        rows = x.reshape(-1, self.in_features).contiguous()
+        rows = x.detach().reshape(-1, self.in_features).contiguous()
         out = self.inner(rows)
         parts = list(out) if isinstance(out, tuple) else [out]
         for i, y in enumerate(parts):

@@ -13,6 +13,7 @@ import threading
 from typing import NamedTuple
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 
@@ -606,6 +607,15 @@ def nvfp4_prepare(w: torch.Tensor, s: torch.Tensor, importance: torch.Tensor | N
 
 
 # ------------------------------------------------------------------------------------------- adapters
+def _outside_autograd(hint: str, names: tuple, *tensors) -> None:
+    """Refuses tensors whose gradient autograd would lose without a word: the results of this module's calls have none."""
+    if torch.is_grad_enabled():
+        for i, t in enumerate(tensors):
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{names[i]} requires a gradient, which autograd does not get through this call: call it in a "
+                                 f"torch.autograd.Function with {hint} in its backward, or under torch.no_grad()")
+
+
 def _fits(t: torch.Tensor, name: str, dtype, shape, dev: int) -> int:
     """The address of a contiguous tensor of this type and shape on device ``dev``."""
     if t.dtype != dtype or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
@@ -735,9 +745,12 @@ def lora(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter: torch.Tenso
     be ``base`` itself; otherwise it overlaps no input.  x, base and out may be column slices of wider matrices.
     K, O and R are multiples of 8, R <= 128, N <= 1024, at most 2^24 rows; adapters of a smaller rank are padded with zeros.
     fp32 sums, one rounding; a row's result does not depend on the other rows' order.  ``workspace``: scratch of the
-    caller's (:func:`lora_workspace`; not shared by calls that may run at the same time), for :func:`read_status`."""
+    caller's (:func:`lora_workspace`; not shared by calls that may run at the same time), for :func:`read_status`.
+    Outside autograd: tensors that require a gradient are refused while gradients are recorded."""
+    _outside_autograd("lora_grad", ("x", "a", "b", "scale", "base", "out"), x, a, b, scale, base, out)
     px, ldx, pa, pb, pi, ps, sizes, dev = _adapter_args(x, a, b, adapter, scale)
     T, O = sizes[0], sizes[2]
+    given = out is not None
     py, ldy, po, ldo, out = _base_and_out(base, out, x, O, T, dev)
     n = _lora_bytes(sizes, 0) if T else 0  # 0 for few rows
     ws, pw = _lora_scratch(workspace, n, x, dev)
@@ -746,6 +759,8 @@ def lora(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter: torch.Tenso
     if po == px:
         raise ValueError("out must not be x")
     _call_on(dev, "pm_lora", px, ldx, pa, pb, pi, ps, py, ldy, po, ldo, *sizes, pw, n)
+    if given:
+        increment_version(out)
     return out
 
 
@@ -759,6 +774,7 @@ def lora_grad(dy: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tenso
     order: the same call gives the same bits.  ``workspace`` as in :func:`lora` (``lora_workspace(..., grad=True)``)."""
     px, ldx, pa, pb, pi, ps, sizes, dev = _adapter_args(x, a, b, adapter, scale)
     T, K, O = sizes[:3]
+    given = out is not None
     pg, _, ldg = _rows(dy, "dy", O, dev, T)
     py, ldy, po, ldo, out = _base_and_out(base, out, x, K, T, dev)
     if T > 0 and (po == px or po == pg):
@@ -768,6 +784,8 @@ def lora_grad(dy: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tenso
     ws, pw = _lora_scratch(workspace, n, x, dev)
     _call_on(dev, "pm_lora_grad", pg, ldg, px, ldx, pa, pb, pi, ps, py, ldy, po, ldo, da.data_ptr(), db.data_ptr(), *sizes,
              pw, n)
+    if given:
+        increment_version(out)
     return out, da, db
 
 
@@ -820,7 +838,9 @@ def router_balance(logits: torch.Tensor, topk_ids: torch.Tensor, valid: torch.Te
     topk_ids [T, k] int32 (:func:`topk`, :func:`router_topk`), over the n live rows: those with ``valid`` [T] (bool,
     None: all) whose logits are not all -inf.  counts[e] = picks of e (ids outside [0, E) are ignored), prob[e] = mean
     softmax probability, loss = E sum_e counts[e] / (k n) prob[e], z_loss = mean logsumexp^2, tokens = n; zeros where no
-    row is live.  Column sums in a fixed order: the same call gives the same bits."""
+    row is live.  Column sums in a fixed order: the same call gives the same bits.  Outside autograd: logits that require a
+    gradient are refused while gradients are recorded."""
+    _outside_autograd("router_grad", ("logits",), logits)
     pl, pi, pv, f32, T, E, k, dev = _router_args(logits, topk_ids, valid)
     f0, i0, f1, i1 = _result_shapes(dev, E)
     loss, z_loss, prob = torch.empty_like(f0), torch.empty_like(f0), torch.empty_like(f1)
@@ -866,10 +886,13 @@ def router_grad(logits: torch.Tensor, topk_ids: torch.Tensor, topk_w: torch.Tens
     dz, dz_dev = _factor(d_z, "d_z", dev)
     if counts is None and (dl != 0.0 or dz != 0.0):
         raise ValueError("d_loss and d_z need counts and tokens")
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty_like(logits)
     po = _fits(out, "out", logits.dtype, (T, E), dev)
     if T == 0:
         return out
     _call_on(dev, "pm_moe_router_grad", pl, f32, pi, pw, pdw, pc, pt, pv, T, E, k, dl, dl_dev, dz, dz_dev, po)
+    if given:
+        increment_version(out)
     return out
