@@ -468,6 +468,11 @@ bool rows_ok(const void* p, int64_t ld, int T, int width, bool written) {
     return a16(p) && ld % 8 == 0 && (T <= 1 || ld >= width || (ld >= 0 && !written));
 }
 
+// A result on top of base has base's row distance, and no result is on top of u or v.
+bool apart(const void* out, int64_t ldout, const void* base, int64_t ldbase, int T, const void* u, const void* v) {
+    return out != u && out != v && (out != base || ldout == ldbase || T <= 1);
+}
+
 int check_lora(int T, int K, int O, int R, int N) {
     if (T < 0 || K <= 0 || O <= 0 || R <= 0 || N <= 0) return PM_ERR_INVALID;
     if (K % 8 || O % 8 || R % 8 || R > kLoraMaxRank || N > kLoraMaxAdapters || T > kLoraMaxRows || K > kLoraMaxWidth ||
@@ -558,6 +563,7 @@ int pm_lora(const void* x, int64_t ldx, const void* a, const void* b, const int3
         (base && !rows_ok(base, ldbase, T, O, false)) || (T > kLoraFewRows && !a16(workspace)))
         return PM_ERR_ALIGN;
     if (workspace_bytes < pm_lora_workspace_bytes(T, K, O, R, N, 0)) return PM_ERR_WORKSPACE;
+    if (!apart(out, ldout, base, ldbase, T, x, x)) return PM_ERR_INVALID;
     int sms = 0;
     if ((st = device_sms(&sms)) != PM_OK) return st;
     cudaStream_t s = (cudaStream_t)stream;
@@ -595,6 +601,7 @@ int pm_lora_grad(const void* dy, int64_t lddy, const void* x, int64_t ldx, const
                   (base && !rows_ok(base, ldbase, T, K, false))))
         return PM_ERR_ALIGN;
     if (workspace_bytes < pm_lora_workspace_bytes(T, K, O, R, N, 1)) return PM_ERR_WORKSPACE;
+    if (T > 0 && !apart(dx, lddx, base, ldbase, T, x, dy)) return PM_ERR_INVALID;
     int sms = 0;
     if ((st = device_sms(&sms)) != PM_OK) return st;
     cudaStream_t s = (cudaStream_t)stream;
