@@ -31,13 +31,21 @@ namespace {
 // {2c, 2c+1, 2c+8, 2c+9} of two steps; both operands are read so, and the sum does not care. In the second product the
 // MMA's column j of tile i is column 8 (j / 2) + 2 i + j % 2 of the piece, so that a lane ends up with 8 neighbours.
 //
-// It runs on the plan's groups where rows x ranks are few, in all or on average for an adapter: every group reads its
-// adapter's weights, and the tiled kernels read them once for 128 rows but work on 128 however few there are. This against
-// the tiled kernels, us replayed, 2048 -> 2048 (rows, rank, adapters): 1000 x 64 of 4 15.8 and 17.3, 4096 x 16 of 64 21.2 and
-// 28.2, 4096 x 64 of 256 65 and 73, 16384 x 16 of 256 69 and 69, of 1024 88 and 202; 5120 x 16 of 4 38 and 32, 8192 x 32 of
-// 128 53 and 44, 4096 x 64 of 128 61 and 47, 2048 x 128 of 64 73 and 47.
+// It runs on the plan's groups where rows x ranks are few, in all or on average for a loaded adapter: every group reads its
+// adapter's weights, and the tiled kernels read them once for 128 rows but work on 128 however few there are. Which adapters have
+// rows the host cannot know, so the rule weighs both ends: rows spread over all adapters / all of one (or 64: the same within a
+// few us). This against the tiled kernels, us replayed, 2048 -> 2048 (rows, rank, adapters):
+//   in all         1000 x 64 of 4 15.8 and 17.3; 4096 x 16 of 64 21 / 19 and 28 / -; 5120 x 16 of 4 38 and 32
+//   256 for each   4096 x 64 of 1024 143 / 43 and 243 / 31; 16384 x 16 of 1024 87 / 67 and 202 / 52
+//   512 for each   2048 x 64 of 256 47 / 22 and 74 / 25; 4096 x 64 of 512 86 / 42 and 130 / 29; 2048 x 128 of 512 171 / 44 and
+//                  232 / 31; 16384 x 32 of 1024 123 / 84 and 212 / 54; 8192 x 64 of 1024 151 / 78 and 249 / 39
+//   640            5120 x 64 of 512 88 / 55 and 131 / 31
+//   1024           4096 x 64 of 256 65 / 41 and 73 / 29; 8192 x 64 of 512 108 / 76 and 133 / 37; 16384 x 64 of 1024 207 / 135 and
+//                  254 / 57; 65536 x 16 of 1024 256 / 217 and 284 / 169; 8192 x 16 of 128 37 / 34 and 41 / 33
+// Up to 512 neither choice loses more than the other where it is the wrong one; beyond, this kernel loses up to 2.4 times on rows
+// of few adapters, and the tiled ones at most 1.5 on spread rows.
 constexpr long kFusedRowRanks = 65536;
-constexpr long kFusedRowRanksEach = 1024;
+constexpr long kFusedRowRanksEach = 512;
 bool lora_fused(int T, int R, int N) { return (long)T * R <= std::max(kFusedRowRanks, kFusedRowRanksEach * N); }
 constexpr int kFewThreads = 256;
 constexpr int kFewWarps = kFewThreads / 32;

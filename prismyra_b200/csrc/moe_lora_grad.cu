@@ -32,7 +32,9 @@ namespace {
 //   512 x 16 of 4 32, 14.7, 21; of 64 spread 12 to 17, 17, 38, all of one 48 to 143, 31, 29
 //   800 x 16 of 4 -, 16.8, 22; of 64 spread -, 18, 39, all of one -, 43, 32
 //   1200 x 16 of 1 -, 25, 26; 2000 x 16 of 4 -, 31, 27
-//   1000 x 16 of 1000 -, 134, 317; 2048 x 16 of 512 spread -, 93, 206, all of one -, 143, 119
+//   1000 x 16 of 1000 -, 134, 317; 2048 x 16 of 512 spread -, 93, 206, all of one -, 131, 119, of 16 -, 51, 113
+//   4096 x 16 of 1024 spread -, 180, 373, all of one -, 292, 219, of 16 -, 100, 221; 1000 x 16 of 256 45, 58 and 29 on groups, 110,
+//   70 and 64 tiled: which adapters have rows the host cannot know, and the groups lose least where they are the wrong choice
 //   32 x 64 of 4 14.8, -, 19; 128 x 64 of 8 22, 25, 20; 1000 x 64 of 16 -, 49, 33: the warps' MMAs take 16 rows at a time, at a
 //   fraction of the tensor core's rate
 constexpr int kGradFewRowRanks = 2048;
