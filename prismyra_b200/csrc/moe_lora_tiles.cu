@@ -666,19 +666,35 @@ constexpr int kUpThreads = 384;   // warps 0-7: base in, results out; 8: MMA; 9:
 __device__ __noinline__ void again(uint8_t* stage, const bf16* h, const bf16* w, int by_rank, int R, int width, int first,
                                    const bf16* base) {
     const int lane = threadIdx.x & 31;
-    const long column = by_rank ? 1 : R, rank = by_rank ? width : 1;
+    auto weights = [&](int j, int r, uint32_t (&v)[8]) {  // column j's ranks r .. r + 7, as the upper halves of fp32
+        if (by_rank) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = (uint32_t)__bfloat16_as_ushort(w[(long)(r + k) * width + first + j]) << 16;
+        } else {
+            const uint4 u = *reinterpret_cast<const uint4*>(w + (long)(first + j) * R + r);
+            v[0] = u.x << 16, v[1] = u.x & 0xffff0000u, v[2] = u.y << 16, v[3] = u.y & 0xffff0000u;
+            v[4] = u.z << 16, v[5] = u.z & 0xffff0000u, v[6] = u.w << 16, v[7] = u.w & 0xffff0000u;
+        }
+    };
+    uint32_t v[8];
     bool inf = false;
     if (first + lane < width)
-#pragma unroll 8
-        for (int r = 0; r < R; ++r)
-            inf |= (__bfloat16_as_ushort(w[(first + lane) * column + r * rank]) & 0x7fffu) == 0x7f80u;
+        for (int r = 0; r < R; r += 8) {
+            weights(lane, r, v);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) inf |= (v[k] & 0x7fffffffu) == 0x7f800000u;
+        }
     for (uint32_t todo = __ballot_sync(0xffffffffu, inf); todo != 0; todo &= todo - 1) {
         const int j = __ffs(todo) - 1;
-        const bf16* p = w + (first + j) * column;
         float s = 0.0f;
-#pragma unroll 8
-        for (int r = 0; r < R; ++r)
-            s = fmaf(__bfloat162float(__ldcg(h + r)), __bfloat162float(p[r * rank]), s);
+        for (int r = 0; r < R; r += 8) {
+            const uint4 u = __ldcg(reinterpret_cast<const uint4*>(h + r));
+            const uint32_t g[4] = {u.x, u.y, u.z, u.w};
+            weights(j, r, v);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                s = fmaf(__uint_as_float(k & 1 ? g[k >> 1] & 0xffff0000u : g[k >> 1] << 16), __uint_as_float(v[k]), s);
+        }
         if (base != nullptr) s += __bfloat162float(__ldcg(base + first + j));
         bf16* o = reinterpret_cast<bf16*>(stage + lane * 64 + (((j >> 3) ^ ((lane >> 1) & 3)) << 4)) + (j & 7);
         if (!finite(__bfloat162float(*o))) *o = __float2bfloat16_rn(s);
