@@ -607,13 +607,12 @@ def nvfp4_prepare(w: torch.Tensor, s: torch.Tensor, importance: torch.Tensor | N
 
 
 # ------------------------------------------------------------------------------------------- adapters
-def _outside_autograd(hint: str, names: tuple, *tensors) -> None:
+def _outside_autograd(hint: str, **tensors) -> None:
     """Refuses tensors whose gradient autograd would lose without a word: the results of this module's calls have none."""
-    if torch.is_grad_enabled():
-        for i, t in enumerate(tensors):
-            if t is not None and t.requires_grad:
-                raise ValueError(f"{names[i]} requires a gradient, which autograd does not get through this call: call it in a "
-                                 f"torch.autograd.Function with {hint} in its backward, or under torch.no_grad()")
+    for name, t in tensors.items():
+        if t is not None and t.requires_grad:
+            raise ValueError(f"{name} requires a gradient, which autograd does not get through this call: call it in a "
+                             f"torch.autograd.Function with {hint} in its backward, or under torch.no_grad()")
 
 
 def _fits(t: torch.Tensor, name: str, dtype, shape, dev: int) -> int:
@@ -719,12 +718,9 @@ def lora_workspace(T: int, K: int, O: int, R: int, N: int, grad: bool = False, d
     return torch.zeros(max(_lora_bytes((T, K, O, R, N), int(grad)), 16), dtype=torch.uint8, device=device or "cuda")
 
 
-def _lora_scratch(workspace: torch.Tensor | None, n: int, x: torch.Tensor, dev: int):
-    """The tensor that holds a call's n bytes of scratch (None: it needs none), and its address. A caller's own begins
-    with the status word, which calls without scratch, whose kernels wait for nothing, leave at 0."""
-    if workspace is None:
-        workspace = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-        return workspace, workspace.data_ptr() if n else None
+def _lora_scratch(workspace: torch.Tensor, n: int, dev: int) -> torch.Tensor:
+    """The caller's tensor for n bytes of scratch. It begins with the status word, which calls without scratch, whose
+    kernels wait for nothing, leave at 0."""
     if workspace.dtype != torch.uint8 or workspace.dim() != 1:
         raise ValueError("workspace must be a uint8 vector")
     at = _fits(workspace, "workspace", torch.uint8, workspace.shape, dev)
@@ -732,7 +728,7 @@ def _lora_scratch(workspace: torch.Tensor | None, n: int, x: torch.Tensor, dev: 
         raise ValueError(f"workspace must hold {max(n, 16)} bytes from a 16-byte boundary on, got {workspace.numel()}")
     if n == 0:
         workspace[:16].zero_()
-    return workspace, at
+    return workspace
 
 
 def lora(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter: torch.Tensor, scale: torch.Tensor | None = None,
@@ -747,18 +743,24 @@ def lora(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter: torch.Tenso
     fp32 sums, one rounding; a row's result does not depend on the other rows' order.  ``workspace``: scratch of the
     caller's (:func:`lora_workspace`; not shared by calls that may run at the same time), for :func:`read_status`.
     Outside autograd: tensors that require a gradient are refused while gradients are recorded."""
-    _outside_autograd("lora_grad", ("x", "a", "b", "scale", "base", "out"), x, a, b, scale, base, out)
+    if torch.is_grad_enabled() and (x.requires_grad or a.requires_grad or b.requires_grad or
+                                    (scale is not None and scale.requires_grad) or
+                                    (base is not None and base.requires_grad) or (out is not None and out.requires_grad)):
+        _outside_autograd("lora_grad", x=x, a=a, b=b, scale=scale, base=base, out=out)
     px, ldx, pa, pb, pi, ps, sizes, dev = _adapter_args(x, a, b, adapter, scale)
     T, O = sizes[0], sizes[2]
     given = out is not None
     py, ldy, po, ldo, out = _base_and_out(base, out, x, O, T, dev)
     n = _lora_bytes(sizes, 0) if T else 0  # 0 for few rows
-    ws, pw = _lora_scratch(workspace, n, x, dev)
+    if workspace is not None:
+        workspace = _lora_scratch(workspace, n, dev)
+    elif n:
+        workspace = torch.empty(n, dtype=torch.uint8, device=x.device)
     if T == 0:
         return out
     if po == px:
         raise ValueError("out must not be x")
-    _call_on(dev, "pm_lora", px, ldx, pa, pb, pi, ps, py, ldy, po, ldo, *sizes, pw, n)
+    _call_on(dev, "pm_lora", px, ldx, pa, pb, pi, ps, py, ldy, po, ldo, *sizes, workspace.data_ptr() if n else None, n)
     if given:
         increment_version(out)
     return out
@@ -781,9 +783,12 @@ def lora_grad(dy: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tenso
         raise ValueError("out must be neither x nor dy")
     da, db = torch.empty_like(a), torch.empty_like(b)
     n = _lora_bytes(sizes, 1)  # 0 for few rows
-    ws, pw = _lora_scratch(workspace, n, x, dev)
+    if workspace is not None:
+        workspace = _lora_scratch(workspace, n, dev)
+    elif n:
+        workspace = torch.empty(n, dtype=torch.uint8, device=x.device)
     _call_on(dev, "pm_lora_grad", pg, ldg, px, ldx, pa, pb, pi, ps, py, ldy, po, ldo, da.data_ptr(), db.data_ptr(), *sizes,
-             pw, n)
+             workspace.data_ptr() if n else None, n)
     if given:
         increment_version(out)
     return out, da, db
@@ -840,7 +845,8 @@ def router_balance(logits: torch.Tensor, topk_ids: torch.Tensor, valid: torch.Te
     softmax probability, loss = E sum_e counts[e] / (k n) prob[e], z_loss = mean logsumexp^2, tokens = n; zeros where no
     row is live.  Column sums in a fixed order: the same call gives the same bits.  Outside autograd: logits that require a
     gradient are refused while gradients are recorded."""
-    _outside_autograd("router_grad", ("logits",), logits)
+    if logits.requires_grad and torch.is_grad_enabled():
+        _outside_autograd("router_grad", logits=logits)
     pl, pi, pv, f32, T, E, k, dev = _router_args(logits, topk_ids, valid)
     f0, i0, f1, i1 = _result_shapes(dev, E)
     loss, z_loss, prob = torch.empty_like(f0), torch.empty_like(f0), torch.empty_like(f1)
