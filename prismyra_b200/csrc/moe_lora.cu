@@ -20,8 +20,8 @@ namespace {
 // pieces of A straight from global memory (mma.sync m16n8k16: what costs here is the operands' way in, and these need no
 // staging), the warps' sums meet in every CTA's shared memory, and each warp then makes its 32-column pieces of the result.
 // One launch, two trips to memory (weights and base of the first piece are asked for before the sums meet), one cluster
-// barrier; many groups at a time keep the memory busy. Bound by latency: replayed, one row 2048 -> 4096 of rank 16 3.9 us, 48
-// rows of 64 adapters 5.5 us (6 MB), 731 rows of rank 8 8.3 us with the plan; where many adapters have a few rows each by how
+// barrier; many groups at a time keep the memory busy. Bound by latency: replayed, one row 2048 -> 4096 of rank 16 4.1 us, 48
+// rows of 64 adapters 5.7 us (6 MB), 731 rows of rank 8 8.6 us with the plan; where many adapters have a few rows each by how
 // well its CTAs' waits overlap: 512 rows of 512 adapters of rank 16 28 us (48 MB), 4096 of 1024 61 us (180 MB).
 //
 // Groups come from the rows' adapters themselves up to kLoraFewRows rows (PLANNED false): a cluster per row, of which the

@@ -55,9 +55,11 @@ __device__ __forceinline__ unsigned part_start(unsigned n, unsigned i, unsigned 
 
 // ------------------------------------------------------------------------------------------- down
 // Warps 0-3 copy the block's rows in and signal each stage themselves, warp 5 brings the weights, warp 4 multiplies: 64 columns
-// a step, about 400 cycles of the issuing thread, 16 KB of rows. Bound by its reads: 26 us for 100 MB (8192 rows, widths 2048
-// and 4096: 3.9 TB/s; 16 us where x comes from L2), 33 us for 134 MB; where rows are few, by latency: 12 us at 5120 rows of
-// 2048, R = 64, 10 MB of weights and 21 MB of rows.
+// a step, about 400 cycles of the issuing thread, 16 KB of rows. Long batches wait for the rows, at 3.9 to 4.1 TB/s, short of what
+// this memory gives (the up kernel reads and writes 5.3 TB/s): 26 us for 100 MB (8192 rows, widths 2048 and 4096; 16 us where x
+// comes from L2), 33 us for 134 MB. Neither the weights nor the MMAs hold it up; that the CTAs are unlike in bytes and one or two to
+// an SM, and that a step takes 128 bytes of rows 4 to 8 KB apart, are likely and not measured apart. Where rows are few, latency: 12
+// us at 5120 rows of 2048, R = 64, 10 MB of weights and 21 MB of rows.
 constexpr int kDownMaxStages = 12;
 constexpr int kDownThreads = 192;    // warps 0-3: rows in, sums out; warp 4: MMA; warp 5: weights by TMA
 constexpr int kDownXBytes = kLoraTile * 128;  // 64 columns of the width per stage
@@ -654,7 +656,8 @@ __device__ void sum_shared_tiles(const OuterArgs& g, const int32_t* units, int c
 // ------------------------------------------------------------------------------------------- up
 // 128 rows x 64 columns a unit, every CTA a run of units, two CTAs to an SM: the products of a unit go into one of two
 // accumulators while the result warps add the other to base, which they fetched two units ahead, and store whole 64-byte
-// pieces of rows. Bound by memory: 84 MB in 17.5 us (5120 rows of 4096: 4.8 TB/s), 134 MB in 25 us (16384 of 2048: 5.3 TB/s).
+// pieces of rows. Bound by memory: 84 MB in 18.5 us (5120 rows of 4096: 4.5 TB/s), 134 MB in 25.5 us (16384 of 2048: 5.3 TB/s), of
+// which looking for results that are not finite takes 0.7.
 constexpr int kUpCols = 64;       // columns of a unit
 constexpr int kUpStages = 3;
 constexpr int kUpThreads = 384;   // warps 0-7: base in, results out; 8: MMA; 9: TMA; 10, 11: rows without an adapter, shared

@@ -7,7 +7,8 @@
 //   c_e = dloss E counts_e / (k n^2)
 // where w are the renormalised top-k weights: w = softmax of the picked logits, so their gradient stays inside the k.
 // Both are one pass over the logits, bound by memory where rows are many: 131072 x 256 fp32, a tenth of it padding, takes the
-// losses 28 us (126 MB, 4.5 TB/s; 141 warp instructions a row) and a finishing launch of 2 us, the gradient 47 us (5.7 TB/s).
+// losses 28 us (126 MB, 4.5 TB/s; 141 warp instructions a row, during which none of its logits are on their way) and a finishing
+// launch of 2 us, the gradient 47 us (5.7 TB/s).
 // 128 x 128 bf16: 4.4 us, in one CTA; 1000 x 128: the gradient 3.7 us.
 //
 // A warp holds a row: lane l owns columns 128 i + 4 l + {0..3} (one 16-byte load of fp32, 8 of bf16) where rows start
@@ -390,8 +391,9 @@ struct GradArgs {
     int T, E, k;
 };
 
-// The top-k terms of a warp's kRowsInFlight rows: lane u KP + j has pick j of row u (KP: k rounded up to a power of two;
-// with KP = 16 the rows take two passes), and puts its term into the row's columns in shared memory.
+// A warp takes kRowsInFlight rows at a time. Of their top-k terms lane u kp + j has pick j of row u (kp: k rounded up to a power of
+// two; with kp = 16 the rows take two passes) and puts its term into the row's columns in shared memory, from where the row's
+// lanes add them as they store.
 template <typename TL, int NV, bool VEC>
 __global__ void __launch_bounds__(kGradThreads, 3)
     router_grad_kernel(const TL* logits, const GradArgs g, TL* dlogits) {  // dlogits may be logits
